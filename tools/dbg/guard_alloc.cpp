@@ -1,10 +1,10 @@
-// guard_alloc.cpp -- a torch.cuda pluggable allocator that puts an UNMAPPED guard range right behind every tensor (debugging aid;
-// VERDICT r5 #2).  Each allocation is its own virtual-memory reservation: `size` rounded up to the mapping granularity is backed
+// guard_alloc.cpp -- a torch.cuda pluggable allocator that puts an UNMAPPED guard range right behind every tensor (debugging aid).
+// Each allocation is its own virtual-memory reservation: `size` rounded up to the mapping granularity is backed
 // by physical memory, one more granule behind it is reserved and never mapped, and the tensor is placed so that it ENDS at the
 // end of the mapped range (start 16-byte aligned: at most 15 bytes of slack).  A kernel that reads or writes 16 bytes past the end
 // of any buffer takes a GPU memory fault at that very launch -- whatever the caching allocator's layout would have hidden.
 //   hipcc -O2 -shared -fPIC -o /tmp/libguard_alloc.so tools/dbg/guard_alloc.cpp
-//   FDGAN_TEST_GUARD_ALLOC=/tmp/libguard_alloc.so AMD_SERIALIZE_KERNEL=3 python -m pytest tests -m gpu ...   (tests/conftest.py)
+//   FDGAN_TEST_GUARD_ALLOC=/tmp/libguard_alloc.so python -m pytest tests -m gpu ...   (tests/conftest.py)
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -34,6 +34,13 @@ long long g_allocs = 0, g_bytes = 0;
   } while (0)
 }  // namespace
 
+// Where a tensor of `size` bytes lies: returns its offset in the mapped range, whose length goes to `mapped` (whole granules).  At the end
+// (16-byte aligned: at most 15 bytes of slack) or at the start.
+extern "C" size_t guard_place(size_t size, size_t gran, int at_end, size_t* mapped) {
+  *mapped = (size + gran - 1) / gran * gran;
+  return at_end ? (*mapped - size) & ~(size_t)15 : 0;
+}
+
 extern "C" void* guard_malloc(ssize_t size, int device, hipStream_t stream) {
   if (size <= 0) return nullptr;
   std::lock_guard<std::mutex> lk(g_mu);
@@ -45,8 +52,13 @@ extern "C" void* guard_malloc(ssize_t size, int device, hipStream_t stream) {
     GCHK(hipMemGetAllocationGranularity(&g_gran, &prop, hipMemAllocationGranularityMinimum));
     fprintf(stderr, "[guard_alloc] granularity %zu bytes\n", g_gran);
   }
+  // GUARD_ALLOC_END=1: the tensor ENDS at the guard (start only 16-byte aligned).  torch's own fills / copies then leave the tail of such
+  // tensors unwritten unless nothing is ever unmapped (GUARD_ALLOC_LEAK=1; results wrong, no fault), so the default places the tensor
+  // at the START of its page-aligned mapping: tensors whose size is a multiple of the 4 KiB granule -- every large power-of-two activation /
+  // gradient buffer, exactly the ones that end at a segment boundary under the caching allocator -- still end exactly at the guard.
+  static const bool at_end = getenv("GUARD_ALLOC_END") != nullptr;
   Rec r;
-  r.mapped = ((size_t)size + g_gran - 1) / g_gran * g_gran;
+  const size_t offset = guard_place((size_t)size, g_gran, at_end, &r.mapped);
   r.reserved = r.mapped + g_gran;
   GCHK(hipMemAddressReserve(&r.va, r.reserved, g_gran, nullptr, 0));
   GCHK(hipMemCreate(&r.h, r.mapped, &prop, 0));
@@ -55,12 +67,7 @@ extern "C" void* guard_malloc(ssize_t size, int device, hipStream_t stream) {
   acc.location = prop.location;
   acc.flags = hipMemAccessFlagsProtReadWrite;
   GCHK(hipMemSetAccess(r.va, r.mapped, &acc, 1));
-  // GUARD_ALLOC_END=1: the tensor ENDS at the guard (start only 16-byte aligned).  Measured round 6: torch's own fills / copies then
-  // leave the tail of such tensors unwritten (results wrong, no fault), so the default places the tensor at the START of its
-  // page-aligned mapping: tensors whose size is a multiple of the 4 KiB granule -- every large power-of-two activation / gradient
-  // buffer, exactly the ones that end at a segment boundary under the caching allocator -- still end exactly at the guard.
-  static const bool at_end = getenv("GUARD_ALLOC_END") != nullptr;
-  char* p = static_cast<char*>(r.va) + (at_end ? ((r.mapped - (size_t)size) & ~(size_t)15) : 0);
+  char* p = static_cast<char*>(r.va) + offset;
   g_live[p] = r;
   ++g_allocs, g_bytes += r.mapped;
   return p;
