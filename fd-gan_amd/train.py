@@ -95,7 +95,7 @@ class TrainStep:
 
     @staticmethod
     def _init_trace(what):
-        """FDGAN_DEBUG_INIT_TRACE=1 (tools/ranks8_loop.sh): drain the device and say on stderr how far this rank's start-up got -- the
+        """FDGAN_DEBUG_INIT_TRACE=1: drain the device and say on stderr how far this rank's start-up got -- the
         last line of a rank that dies names the phase whose GPU work raised the abort (profiles/r6_oversubscription.txt)."""
         if os.environ.get("FDGAN_DEBUG_INIT_TRACE"):
             import sys
