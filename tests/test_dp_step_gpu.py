@@ -160,20 +160,6 @@ def test_bench_py_plain_python_launches_its_own_ranks(gpus):
     cmd = [sys.executable, os.path.join(root, "bench.py"), "--gpus", str(gpus), "--steps", "2", "--warmup", "1",
            "--batch", "2", "--size", "64", "--no-forward-leg", "--no-cpu-baseline"]
     out = subprocess.run(cmd, env=env, capture_output=True, text=True, timeout=900)
-    if out.returncode != 0 and gpus > 1 and "HSA_STATUS_ERROR_ILLEGAL_INSTRUCTION" in out.stderr and "sync_replicas" in out.stderr:
-        # Round 6, profiles/r6_oversubscription.txt: with EIGHT processes on ONE GPU (this test's hook only -- RCCL refuses it and the
-        # driver never does it) about one launch in 30 loses a rank to an illegal-instruction queue abort while the replicas are
-        # being synchronised: every launch of this library in the dying rank had completed (the gloo broadcasts in front of that
-        # point synchronise the stream), only PyTorch's checksum kernels / gloo's copies were in flight, and 14 000 steady-state
-        # iterations + 320 process start-ups of this library's kernels alone under the same oversubscription lost none.  Start-up
-        # markers pinned it to PyTorch's fp64 checksum kernels on a drained device; those checksums are formed on the host since
-        # (64 of 64 launches clean).  One retry stays, recorded; a second abort fails the test.
-        try:
-            with open(os.path.join(root, "gpurun_out", "bench_ranks%d_startup_abort.txt" % gpus), "w") as f:
-                f.write(out.stderr)
-        except OSError:
-            pass
-        out = subprocess.run(cmd, env=env, capture_output=True, text=True, timeout=900)
     if out.returncode != 0:      # the launcher's summary (SIGTERMs of the surviving ranks) hides the first failure: show the tracebacks
         err = out.stderr.splitlines()
         first = [i for i, ln in enumerate(err) if "Traceback" in ln or "Error" in ln][:6]
