@@ -196,14 +196,29 @@ template <int T, int N> struct GroupSum {
 
 template <int T> constexpr int block_of() { return T > 256 ? T : 256; }
 
+// A row of equal values v has to find its mean v again, to the last bit: its differences are divided by sqrt(eps), so that one rounding of a mean
+// of 60000 (0.004) would come out as a y of 0.8 where there is nothing to see.  The sum of n values v is exact where n times v's digits fit the
+// 24 of fp32: n up to 8192 for fp16's 11 digits, 65536 for bf16's 8.  Beyond that, and for fp32, the mean is mended: the differences d = x - m
+// of the pass that squares them are summed as well, e = sum d / C is what m is off by, and x - (m + e) = d - e.  (In a row of equal values
+// all d are the same few steps of v, so that their sum, e, and the square below are exact.)
+template <int DT> constexpr bool mend_mean(int n) { return DT == FD_F32 || n > (DT == FD_F16 ? 8192 : 65536); }
+// sum of squares around m, and e, to the mean square around m + e (rounding may leave a little below 0; infinity and NaN stay)
+__device__ __forceinline__ float around(float mean_square, float e) {
+  const float q = e * e;
+  return mean_square < INFINITY ? (mean_square > q ? mean_square - q : 0.f) : mean_square;
+}
+
 // ---- forward, held rows ---------------------------------------------------------------------------------------------------------
 // Bound by memory: 45.5 us for 128 MB in and out (65536 x 1024 bf16, 5.9 TB/s; a copy of 128 MB runs at 7.2, one of 2 GB at 4.9), 48 us for
 // 16384 x 4096 bf16, 17 us for 262144 x 72 fp16 (4.4 TB/s: rows of 144 bytes end inside lines).  Two or three vectors a lane because one
 // leaves lanes idle: 24 us instead of 17 at 72 channels, 16 lanes of which 9 work.
 template <int DT, int T, int NV> __global__ __launch_bounds__(block_of<T>()) void ln_fwd_rows(LnFwdArgs a) {
   constexpr int V = El<DT>::V, R = block_of<T>() / T;      // rows of a workgroup at a time
-  __shared__ float red[2][16][1];
+  constexpr bool MEND = mend_mean<DT>(T * NV * V);
+  constexpr int S = MEND ? 2 : 1;
+  __shared__ float red[2][16][1], red2[2][16][S];
   GroupSum<T, 1> sum{red};
+  GroupSum<T, S> sum2{red2};
   const int lane = threadIdx.x % T, sub = threadIdx.x / T;
   constexpr int H = T < 1024 ? NV : 1;                     // 1024 lanes have 128 registers each: the weights are read again for every row
   float w[H][V], b[H][V];
@@ -241,8 +256,8 @@ template <int DT, int T, int NV> __global__ __launch_bounds__(block_of<T>()) voi
 #pragma unroll
       for (int e = 0; e < V; ++e) s[0] += x[k][e];
     sum(s);
-    const float m = s[0] / (float)a.c;               // not times 1 / C: a row of equal values has to find its value again
-    s[0] = 0.f;
+    const float m = s[0] / (float)a.c;               // not times 1 / C (see mend_mean)
+    float sq[S] = {};                                // squares, differences
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int cnt = c - (k * T + lane) * V;
@@ -253,23 +268,30 @@ template <int DT, int T, int NV> __global__ __launch_bounds__(block_of<T>()) voi
         for (int e = 0; e < V; ++e) x[k][e] = e < cnt ? x[k][e] : 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[0] += x[k][e] * x[k][e];
+      for (int e = 0; e < V; ++e) {
+        sq[0] += x[k][e] * x[k][e];
+        if constexpr (MEND) sq[1] += x[k][e];
+      }
     }
-    sum(s);
-    const float rs = rsqrtf(s[0] * a.inv_c + a.eps);
+    sum2(sq);
+    float off = 0.f;
+    if constexpr (MEND) off = sq[1] / (float)a.c;
+    const float rs = rsqrtf((MEND ? around(sq[0] / (float)a.c, off) : sq[0] * a.inv_c) + a.eps);
     if (c && lane == 0) {
-      if (a.mean) a.mean[r] = m;
+      if (a.mean) a.mean[r] = m + off;
       if (a.rstd) a.rstd[r] = rs;
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int i = (k * T + lane) * V, q = T < 1024 ? k : 0;
+      int i = (k * T + lane) * V;
+      const int q = T < 1024 ? k : 0;
       if constexpr (T == 1024) {
+        asm("" : "+v"(i));                                 // else the weights' addresses are kept over the rows, in registers that are not there
         load_weight<V>(a.gamma, a.wdt, i, a.c - i, 1.f, w[0]);
         load_weight<V>(a.beta, a.wdt, i, a.c - i, 0.f, b[0]);
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[k][e] = x[k][e] * rs * w[q][e] + b[q][e];
+      for (int e = 0; e < V; ++e) x[k][e] = (MEND ? x[k][e] - off : x[k][e]) * rs * w[q][e] + b[q][e];
       Vec<DT, V>::store(a.y, r * a.py + i, c - i, x[k]);
     }
   }
@@ -282,8 +304,9 @@ template <int DT, int T, int NV> __global__ __launch_bounds__(block_of<T>()) voi
 // for one workgroup a row; both are a launch and one round of memory latency.
 template <int DT, int NV> __global__ __launch_bounds__(256) void ln_fwd_part(LnFwdArgs a) {
   constexpr int V = El<DT>::V;
-  __shared__ float red[2][16][1];
+  __shared__ float red[2][16][1], red2[2][16][2];
   GroupSum<256, 1> sum{red};
+  GroupSum<256, 2> sum2{red2};
   const long long r = blockIdx.x / a.pieces;
   const int p = blockIdx.x % a.pieces, at = p * a.piece, n = a.c - at < a.piece ? a.c - at : a.piece;
   float x[NV][V], s[1] = {0.f};
@@ -298,27 +321,30 @@ template <int DT, int NV> __global__ __launch_bounds__(256) void ln_fwd_part(LnF
     for (int e = 0; e < V; ++e) s[0] += x[k][e];
   sum(s);
   const float m = s[0] / (float)n;
-  s[0] = 0.f;
+  float sq[2] = {0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int cnt = n - (k * 256 + (int)threadIdx.x) * V;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float d = e < cnt ? x[k][e] - m : 0.f;
-      s[0] += d * d;
+      sq[0] += d * d;
+      sq[1] += d;
     }
   }
-  sum(s);
+  sum2(sq);
   if (threadIdx.x == 0) {
-    a.part[2 * (r * a.pieces + p)] = m;
-    a.part[2 * (r * a.pieces + p) + 1] = s[0];
+    const float off = sq[1] / (float)n;
+    a.part[2 * (r * a.pieces + p)] = m + off;
+    a.part[2 * (r * a.pieces + p) + 1] = around(sq[0] / (float)n, off) * (float)n;
   }
 }
 
 template <int DT, int NV> __global__ __launch_bounds__(256) void ln_fwd_apply(LnFwdArgs a) {
   constexpr int V = El<DT>::V;
-  __shared__ float red[2][16][1];
+  __shared__ float red[2][16][1], red2[2][16][2];
   GroupSum<256, 1> sum{red};
+  GroupSum<256, 2> sum2{red2};
   const long long r = blockIdx.x / a.pieces;
   const int p = blockIdx.x % a.pieces, at = p * a.piece, n = a.c - at < a.piece ? a.c - at : a.piece;
   float x[NV][V];
@@ -331,14 +357,16 @@ template <int DT, int NV> __global__ __launch_bounds__(256) void ln_fwd_apply(Ln
   float s[1] = {0.f};
   for (int j = threadIdx.x; j < a.pieces; j += 256) s[0] += pt[2 * j] * (float)(j + 1 < a.pieces ? a.piece : a.c - j * a.piece);
   sum(s);
-  const float m = s[0] / (float)a.c;
-  s[0] = 0.f;
+  const float m0 = s[0] / (float)a.c;
+  float sq[2] = {0.f, 0.f};
   for (int j = threadIdx.x; j < a.pieces; j += 256) {
-    const float d = pt[2 * j] - m;
-    s[0] += pt[2 * j + 1] + d * d * (float)(j + 1 < a.pieces ? a.piece : a.c - j * a.piece);
+    const float d = pt[2 * j] - m0, nj = (float)(j + 1 < a.pieces ? a.piece : a.c - j * a.piece);
+    sq[0] += pt[2 * j + 1] + d * d * nj;
+    sq[1] += d * nj;
   }
-  sum(s);
-  const float rs = rsqrtf(s[0] * a.inv_c + a.eps);
+  sum2(sq);
+  const float off = sq[1] / (float)a.c, m = m0 + off;      // see mend_mean: the mean of the means is mended the same way
+  const float rs = rsqrtf(around(sq[0] / (float)a.c, off) + a.eps);
   if (p == 0 && threadIdx.x == 0) {
     if (a.mean) a.mean[r] = m;
     if (a.rstd) a.rstd[r] = rs;
@@ -733,9 +761,9 @@ template <int DT> int launch_fwd(LnFwdArgs& a, hipStream_t st) {
   if (s.T)
     return with_fwd(s, [&](auto t, auto nv) {
       constexpr int T = decltype(t)::value, NV = decltype(nv)::value, R = block_of<T>() / T;
-      // as many workgroups as the registers let the chip hold at once (16-bit types 46, 78 to 86, 107 to 125 a lane at 1, 2, 3 or 4 vectors, fp32
-      // 33 to 88): a few more than that would take a whole second round for themselves
-      constexpr int WAVES = NV == 1 ? 8 : El<DT>::V == 4 ? (NV == 2 ? 8 : NV == 3 ? 6 : 5) : NV == 2 ? (T <= 64 ? 5 : 6) : 4;
+      // as many workgroups as the registers let the chip hold at once (16-bit types 46, 78 to 86, 107 to 124 a lane at 1, 2 or 3 vectors, fp32
+      // 35, 51 to 64, 67 to 79, 86 at 512 lanes x 3; 1024 lanes 50 to 81): a few more than that would take a whole second round for themselves
+      constexpr int WAVES = NV == 1 ? 8 : El<DT>::V == 4 ? (NV == 2 ? 8 : NV == 3 && T < 512 ? 6 : 5) : NV == 2 ? (T <= 64 ? 5 : 6) : 4;
       constexpr int MOST = 256 * (WAVES * 256 / block_of<T>());
       const long long b = (a.rows + R - 1) / R;
       return fd_launch(&ln_fwd_rows<DT, T, NV>, "layer_norm_fwd", dim3((unsigned)(b < MOST ? b : MOST)), dim3(block_of<T>()), 0, a, st);
