@@ -384,7 +384,7 @@ template <int DT, int NV> __global__ __launch_bounds__(256) void ln_fwd_apply(Ln
 }
 
 // ---- backward, held rows --------------------------------------------------------------------------------------------------------
-// An element that does not exist has dy = 0 and so adds nothing anywhere.  What waits for a row's two sums are the vectors as they were
+// An element that does not exist has dy = 0 and h = 0 and so adds nothing anywhere.  What waits for a row's two sums are the vectors as they were
 // loaded, converted a second time: half the registers of the converted ones, which is what decides how many waves a CU holds.
 // 82 us for 16384 x 4096 bf16 (402 MB, 4.9 TB/s: a large copy's rate), 52 us for 262144 x 144 fp16 (4.4 TB/s).
 // Rows of T lanes: one vector a lane up to 512 of them (few registers, many waves), two or three only where a row takes all 512.
@@ -426,7 +426,7 @@ template <int DT, int GT, int T, int NV, int V> __global__ __launch_bounds__(T *
   for (long long r0 = (long long)blockIdx.x * R; r0 < a.rows; r0 += hop) {
     const long long r = r0 + sub;
     const int c = r < a.rows ? a.c : 0;
-    const float rs = rn, mrs = -mn * rn;                   // h = x rs - m rs, fused: off by half a step of m rs, as m itself is
+    const float rs = rn, m = mn;                           // h = (x - m) rs: a fused x rs - m rs would leave m rs's rounding where x is m
     typename X::raw_t xr[NV];
     typename Y::raw_t gr[NV];
     float s[2] = {0.f, 0.f};
@@ -438,9 +438,14 @@ template <int DT, int GT, int T, int NV, int V> __global__ __launch_bounds__(T *
       float x[V], g[V];
       X::open(xr[k], x);
       Y::open(gr[k], g);
+      const int cnt = c - (k * T + lane) * V;
+      if (cnt < V) {                                       // what does not exist has h = 0: 0 times an infinite m rs would be NaN
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = e < cnt ? x[e] : m;
+      }
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float h = fmaf(x[e], rs, mrs), t = g[e] * w[k][e];
+        const float h = (x[e] - m) * rs, t = g[e] * w[k][e];
         db[k][e] += g[e];
         dw[k][e] = fmaf(g[e], h, dw[k][e]);
         s[0] += t;
@@ -458,7 +463,7 @@ template <int DT, int GT, int T, int NV, int V> __global__ __launch_bounds__(T *
         X::open(xr[k], x);
         Y::open(gr[k], g);
 #pragma unroll
-        for (int e = 0; e < V; ++e) g[e] = fmaf(g[e] * w[k][e], rs, fmaf(fmaf(x[e], rs, mrs), c2, c1));
+        for (int e = 0; e < V; ++e) g[e] = fmaf(g[e] * w[k][e], rs, fmaf((x[e] - m) * rs, c2, c1));
         Y::store(a.dx, r * a.pdx + i, c - i, g);
       }
     }
@@ -561,7 +566,7 @@ template <int DT, int GT, int NV> __global__ __launch_bounds__(256) void ln_bwd_
     for (int e = 0; e < V; ++e) {
       const float t = g[e] * w[e];
       s[0] += t;
-      s[1] += t * ((h[e] - m) * rs);
+      s[1] += t * (i + e < n ? (h[e] - m) * rs : 0.f);
     }
   }
   sum(s);
@@ -691,7 +696,7 @@ Shape shape_bwd(long long rows, long long c, int V) {
   if (s.T) {
     const int R = s.T > 256 ? 1 : s.T > 128 ? 2 : s.T == 128 ? 4 : 512 / s.T;
     const long long b = (rows + R - 1) / R;
-    // what the registers let the chip hold at once: 87 to 93 a lane at one vector of 8, 146 and 208 at two and three
+    // what the registers let the chip hold at once: 85 to 97 a lane at one vector of 8, 146 and 206 at two and three
     const int most = s.NV > 1 && s.V > 4 ? 256 : 512;
     s.blocks = (int)(b < most ? b : most);      // (768 at one vector: 97 us instead of 83 at 16384 x 4096 bf16, a second round half empty)
     s.floats = 2ll * s.blocks * s.stride;
