@@ -168,6 +168,9 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
 
 Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& shape, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
   TORCH_CHECK(entries.fwd, "fdgan::layer_norm: the library's entries are not bound (fdgan_hip.lib.torch_ops)");
+  // a tangent would be dropped: below, only requires_grad is asked for
+  const auto dual = [](const std::optional<Tensor>& t) { return t && t->defined() && t->_fw_grad(0).defined(); };
+  TORCH_CHECK(!x._fw_grad(0).defined() && !dual(weight) && !dual(bias), "layer_norm: forward-mode derivatives are not offered (the gradient is, once)");
   TORCH_CHECK(x.is_cuda(), "layer_norm: the FD-GAN HIP path needs a tensor on an MI355X (`cuda`) device; there is no CPU fallback");
   const int64_t k = (int64_t)shape.size(), lead = x.dim() - k;
   TORCH_CHECK_VALUE(k > 0 && lead >= 0 && x.sizes().slice(lead) == at::IntArrayRef(shape), "layer_norm: a tensor of shape ", x.sizes(),

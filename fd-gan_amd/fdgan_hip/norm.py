@@ -6,7 +6,8 @@ the BatchNorm that the planned networks fold into their convolutions.
 
 x: fp32, fp16 or bf16 on the GPU; the result has its shape and type and is contiguous.  weight / bias: fp32 or x's type.  Statistics and
 sums are fp32 whatever the types; every result is rounded once.  A row may lie in a wider buffer (the leading dimensions at one
-pitch: a channel slice of a concatenation); any other layout is copied first.  Gradients can be taken once."""
+pitch: a channel slice of a concatenation); any other layout is copied first.  Gradients can be taken once; forward-mode derivatives
+(torch.autograd.forward_ad, torch.func.jvp) are refused."""
 import numbers
 
 import torch
@@ -18,7 +19,7 @@ _op = None
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     """torch.nn.functional.layer_norm(x, normalized_shape, weight, bias, eps) on the HIP path.  ValueError for shapes that do not fit and a
-    negative eps, TypeError for other types, RuntimeError off the GPU (csrc/torch_ops.cpp)."""
+    negative eps, TypeError for other types, RuntimeError off the GPU and for tensors with a forward-mode tangent (csrc/torch_ops.cpp)."""
     global _op
     if _op is None:
         _op = L.torch_ops().layer_norm.default

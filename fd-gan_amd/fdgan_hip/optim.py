@@ -26,7 +26,7 @@ def _norm_kind(norm_type, what):
 
 def grad_norm(tensors, norm_type=2.0):
     """The norm of all elements of all `tensors` (an iterable of fp32 / fp16 / bf16 tensors of one GPU, or one tensor) as if they were one
-    vector: norm_type 1, 2 or inf.  An empty list has norm 0."""
+    vector: norm_type 1, 2 or inf.  An empty list has norm 0.  No derivative passes through it."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     return L.torch_ops().grad_norm(tensors, _norm_kind(norm_type, "grad_norm"))
 
