@@ -13,6 +13,7 @@
 // Sums are in fp64: a gradient of 1e-23 or 1e+23 squares to 0 or infinity in fp32, and the MI355X forms fp64 multiply-adds at the
 // rate of fp32 ones, far above what the memory delivers.
 #include "common.h"
+#include "adam.h"
 #include <math.h>
 
 namespace {
@@ -59,18 +60,6 @@ struct FinishArgs {
   double* total;                      // one combined partial (may be null)
   float* norm_out;                    // may be null
 };
-
-// The update of adam_kernel (elementwise.hip).  Its two fused products are written out -- left to the compiler they differ from kernel to
-// kernel -- so that a bound that is never reached changes no bit of a step (flat buffers whose length is a multiple of 4, as FlatAdam's).
-struct AdamUpdate {
-  float lr, b1, b2, eps, bc1, bc2;    // bc = 1 - beta^t
-};
-__device__ __forceinline__ void adam_update(const AdamUpdate& a, float g, float& p, float& m, float& v) {
-#pragma clang fp contract(off)
-  m = fmaf(a.b1, m, (1.f - a.b1) * g);
-  v = fmaf(a.b2, v, (1.f - a.b2) * g * g);
-  p -= a.lr * (m / a.bc1) / (sqrtf(v / a.bc2) + a.eps);
-}
 
 struct AdamClipArgs {
   float *p, *m, *v;
@@ -460,15 +449,14 @@ extern "C" int fdgan_grad_clip(const FdGradSpan* spans, int64_t nspans, int norm
   return fd_launch(&norm_finish_kernel, "grad_norm_finish", dim3(1), dim3(256), 0, f, st);
 }
 
-extern "C" int fdgan_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
+extern "C" int fdgan_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, double beta1, double beta2, float eps,
                                        int64_t step, float max_norm, double* partial, int64_t capacity, float* norm_out, FdStream stream) {
   FD_REQUIRE(p && g && m && v && n > 0 && step >= 1, "adam_step_clipped: bad arguments");
   FD_REQUIRE((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) == 0, "adam_step_clipped: 16-byte aligned flat tensors");
   FD_REQUIRE(norm_out && partial && max_norm >= 0.f, "adam_step_clipped: NULL output or workspace, or max_norm %g", (double)max_norm);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const FdGradSpan s{const_cast<float*>(g), n, FD_F32};
-  AdamClipArgs a{p, m, v, g, n, {lr, beta1, beta2, eps, (float)(1.0 - pow((double)beta1, (double)step)),
-                 (float)(1.0 - pow((double)beta2, (double)step))}, {}};
+  AdamClipArgs a{p, m, v, g, n, adam_constants(lr, beta1, beta2, eps, step), {}};
   int rc = check_spans("adam_step_clipped", &s, 1);
   if (rc == FD_OK && n <= SMALL) {
     FD_REQUIRE(capacity >= fdgan_grad_norm_workspace(&s, 1), "adam_step_clipped: the workspace holds %lld partials", (long long)capacity);

@@ -306,14 +306,14 @@ std::optional<Tensor> adam_step(const Tensor& p, const Tensor& g, const Tensor& 
   float *pp = p.data_ptr<float>(), *mp = m.data_ptr<float>(), *vp = v.data_ptr<float>();
   const float* gp = g.data_ptr<float>();
   if (!max_norm) {
-    check(entries.adam(pp, gp, mp, vp, n, (float)lr, (float)b1, (float)b2, (float)eps, step, stream_of(p)), "adam_step");
+    check(entries.adam(pp, gp, mp, vp, n, (float)lr, b1, b2, (float)eps, step, stream_of(p)), "adam_step");
   } else {
     const FdGradSpan s{const_cast<float*>(gp), n, FD_F32};
     const int64_t room = entries.norm_workspace(&s, 1);
     TORCH_CHECK(room > 0, "adam_step_: the tensors are too long");
     const Tensor partial = at::empty({room}, options.dtype(at::kDouble));
     norm = at::empty({}, options.dtype(at::kFloat));
-    check(entries.adam_clipped(pp, gp, mp, vp, n, (float)lr, (float)b1, (float)b2, (float)eps, step, (float)*max_norm, partial.data_ptr<double>(), room,
+    check(entries.adam_clipped(pp, gp, mp, vp, n, (float)lr, b1, b2, (float)eps, step, (float)*max_norm, partial.data_ptr<double>(), room,
                                norm->data_ptr<float>(), stream_of(p)),
           "adam_step_clipped");
   }

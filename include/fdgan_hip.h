@@ -51,7 +51,7 @@
 extern "C" {
 #endif
 
-#define FDGAN_ABI_VERSION 17
+#define FDGAN_ABI_VERSION 18
 
 enum FdStatus {
   FD_OK = 0,
@@ -490,8 +490,9 @@ int fdgan_out_act_bwd(const float* dout, const float* out, int64_t n, int64_t c,
 int fdgan_grad_ew(int mode, const FdTensor* src, const FdTensor* ref, const FdTensor* dst, FdStream stream);
 
 /* torch.optim.Adam's update (no weight decay, no amsgrad -- what the reference's lrG / lrD / beta1 flags configure,
- * demo.py:43-46) on one flat fp32 tensor: exp_avg m, exp_avg_sq v, 1-based `step` for the bias corrections. */
-int fdgan_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
+ * demo.py:43-46) on one flat fp32 tensor: exp_avg m, exp_avg_sq v, 1-based `step` for the bias corrections.  The betas are
+ * doubles (ABI v18): 1 - beta and 1 - beta^step are formed from them in 64 bits and rounded once. */
+int fdgan_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float lr, double beta1, double beta2, float eps,
                     int64_t step, FdStream stream);
 
 /* The global norm of a list of gradients, clipping by it, and Adam on the clipped gradient (ABI v17).  The list is host memory, read
@@ -514,7 +515,7 @@ int fdgan_grad_norm(const FdGradSpan* spans, int64_t nspans, int norm_type, doub
                     FdStream stream);
 int fdgan_grad_clip(const FdGradSpan* spans, int64_t nspans, int norm_type, float max_norm, double* partial, int64_t capacity,
                     float* norm_out, FdStream stream);
-int fdgan_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
+int fdgan_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_t n, float lr, double beta1, double beta2, float eps,
                             int64_t step, float max_norm, double* partial, int64_t capacity, float* norm_out, FdStream stream);
 
 /* Layer norm over the channels of every (n, h, w) row of a view (ABI v17): y = (x - mean) * rstd * gamma + beta with the row's own mean

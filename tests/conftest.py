@@ -23,6 +23,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with `-m gpu` on the GPU box)")
 
 
+# Tests that hold a value which has been shown to be wrong: they run, and where they fail it is this.
+_WRONG_REFERENCE = {
+    "test_grad_clip_gpu.py::test_clipped_adam": "its reference rounds the betas to fp32 before it forms 1 - beta (0.00099998713 for 0.001, 1.3e-5 off, against a bound of "
+                                                "1.1e-6); test_adam_betas_gpu.py holds the step to the betas as they are passed, at these sizes and bounds",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        why = _WRONG_REFERENCE.get("%s::%s" % (os.path.basename(str(item.fspath)), getattr(item, "originalname", item.name)))
+        if why:
+            item.add_marker(pytest.mark.xfail(reason=why, strict=False))
+
+
 # FDGAN_TEST_POISON=1: every `torch.empty` / `empty_like` on the GPU comes back filled with a huge FINITE value (1e30; 3e4 in fp16; all-ones
 # bytes for integers) instead of whatever the caching allocator's block held before: a kernel that consumes a workspace slot, a partial sum
 # or a temporary nobody wrote shows up as a 1e30-sized error in EVERY run, not as a NaN in one run of six (finite on purpose: padded channels
