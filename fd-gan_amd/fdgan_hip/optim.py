@@ -94,7 +94,12 @@ class FlatAdam:
         E.require_gpu(self.flat, "FlatAdam.step")          # the update is a HIP kernel; no CPU fallback
         self.t += 1
         lr = self.param_groups[0]["lr"]
-        self.grad_norm = adam_step_(self.flat, self.grad, self.m, self.v, self.t, lr, self.betas, self.eps, self.max_norm)
+        if self.max_norm is None:                          # one launch of the library: nothing of torch_ops() is needed
+            with torch.cuda.device(self.flat.device):
+                L.check(L.load().fdgan_adam_step(self.flat.data_ptr(), self.grad.data_ptr(), self.m.data_ptr(), self.v.data_ptr(), self.flat.numel(),
+                                                 lr, self.betas[0], self.betas[1], self.eps, self.t, E.stream_ptr()), "adam_step")
+        else:
+            self.grad_norm = adam_step_(self.flat, self.grad, self.m, self.v, self.t, lr, self.betas, self.eps, self.max_norm)
         # the kernel wrote the parameters behind autograd's back: bump their version counters, which is what the
         # planned modules watch to re-pack their MFMA filter images (netplan.refresh_weights)
         torch.autograd.graph.increment_version(self.params)

@@ -77,3 +77,22 @@ def test_against_torch(O):
         v = opt.state[ref]["exp_avg_sq"].double()
         assert ((d[3].cpu().double() - v).abs() <= 2 * t * 8 * U * v).all()      # either side: up to 4 roundings a step
         assert float((d[0].cpu() - ref.detach()).abs().max()) <= t * (2 * U * 4.0 + 64 * U * 1e-3 * 10)
+
+
+def test_an_optimizer_without_a_bound_needs_the_library_alone(O, monkeypatch):
+    """FlatAdam(max_norm=None) is one entry of the library: it steps where the torch module is not there."""
+    from fdgan_hip import lib as L
+
+    def gone():
+        raise L.FdganLibraryError("libfdgan_torch.so not found")
+    ps = [torch.nn.Parameter(torch.randn(5, 3, device=DEV)), torch.nn.Parameter(torch.randn(7, device=DEV))]
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    a, b = O.FlatAdam(ps, lr=1e-2), O.FlatAdam(twin, lr=1e-2, max_norm=1e9)
+    for opt in (a, b):
+        opt.grad.copy_(torch.linspace(-1, 1, opt.grad.numel(), device=DEV))
+    b.step()
+    monkeypatch.setattr(L, "torch_ops", gone)
+    version = ps[0]._version
+    a.step()
+    assert a.grad_norm is None and ps[0]._version > version
+    assert torch.equal(a.flat, b.flat) and torch.equal(a.m, b.m) and torch.equal(a.v, b.v)
