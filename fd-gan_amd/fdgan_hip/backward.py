@@ -118,6 +118,39 @@ def _overlap(a, b):
     return a[0] == b[0] and a[1] < b[2] and b[1] < a[2]
 
 
+def _reads(r):
+    v = r.get("x") if r["kind"] == "conv" else r.get("src")
+    return _region(v) if v is not None and hasattr(v, "buf") else None
+
+
+def _writes(r):
+    v = r.get("y") if r["kind"] == "conv" else r.get("dst")
+    return _region(v) if v is not None and hasattr(v, "buf") else None
+
+
+def sole_reader(recs, i):
+    """Whether record i is the only one that reads its source between the record that wrote it and the next that writes over it: then the
+    source's gradient is record i's alone."""
+    rx = _reads(recs[i])
+    hits = lambda region: region is not None and _overlap(region, rx)  # noqa: E731
+    prod = next((j for j in range(i - 1, -1, -1) if hits(_writes(recs[j]))), -1)
+    nxt = next((k for k in range(i + 1, len(recs)) if hits(_writes(recs[k]))), len(recs))
+    return not any(t != i and hits(_reads(recs[t])) for t in range(prod + 1, nxt))
+
+
+def layer_norm_sources(recs):
+    """{index of a layer norm's record: sole_reader}.  Its backward pass reads the source again: one that a later op overwrites is refused."""
+    out = {}
+    for i, r in enumerate(recs):
+        if r["kind"] != "layer_norm":
+            continue
+        rx = _reads(r)
+        if any(_writes(q) is not None and _overlap(_writes(q), rx) for q in recs[i + 1:]):
+            raise NotImplementedError("backward of a layer norm whose source a later op of the plan overwrites")
+        out[i] = sole_reader(recs, i)
+    return out
+
+
 class _InPlace:
     """Marker in a `grads` dict: the gradient was accumulated straight into the parameter's own `.grad` (a view of an
     optimizer's flat gradient buffer, see optim.FlatAdam); the autograd bridge returns None for it."""
@@ -175,6 +208,7 @@ class PlanBackward:
     def __init__(self, plan):
         self.plan = plan
         self.recs = plan.records
+        self.norm_sole = layer_norm_sources(self.recs)
         self.gbuf = {}          # activation buffer data_ptr -> gradient buffer
         self.multi_version = set()
         alias = getattr(plan, "grad_alias", {})
@@ -1064,12 +1098,20 @@ class PlanBackward:
                 self.flush(r["dst"])
                 E.mul_mask(r["mask"], self.G(r["dst"]), r["up2"])
                 continue
-            if r["kind"] == "layer_norm":   # the source's gradient has this one writer: stored
+            if r["kind"] == "layer_norm":
                 self.flush(r["dst"])
                 ln = r["ln"]
                 dw, db = (grad_target(grads, p) if p is not None and p.requires_grad else None for p in (ln.weight, ln.bias))
                 ws = self.persistent(("layer_norm", i), lambda: torch.empty(E.layer_norm_workspace(r["src"], True), dtype=torch.float32, device=self.plan.device))
-                E.layer_norm_bwd(r["src"], ln, r["stats"], self.G(r["dst"]), self.G(r["src"]), dw, db, ws)
+                gx = self.G(r["src"])
+                # stored where this op alone contributes to the source's gradient, else added to what the others have put there
+                if self.norm_sole[i] and r["src"].buf.data_ptr() not in self.multi_version and not (
+                        head is not None and _overlap(_region(head[0]["x"]), _region(r["src"]))):
+                    E.layer_norm_bwd(r["src"], ln, r["stats"], self.G(r["dst"]), gx, dw, db, ws)
+                else:
+                    t = self.persistent(("layer_norm_dx", i), lambda: E.new_grad(*r["src"].shape[:3], _r8(r["src"].c), self.plan.device, zero=True))
+                    E.layer_norm_bwd(r["src"], ln, r["stats"], self.G(r["dst"]), E.View(t, 0, r["src"].c), dw, db, ws)
+                    E.grad_ew(E.GRAD_ADD, E.View(t, 0, r["src"].c), gx)
                 self._hook(i)
                 continue
             if r["kind"] in ("pyramid", "bn_dropout", "maxpool3"):      # the legacy DCPDN networks' own ops (csrc/legacy_bwd.hip)

@@ -139,7 +139,9 @@ class NetPlan:
 
     def layer_norm(self, src, dst, ln):
         """dst = layer norm over each pixel's channels of `src`, with module `ln` (fdgan_hip.norm.LayerNorm over the channels): a tensor of its
-        own, because a pixel's mean and variance are no per-channel scale and shift that the next conv's prologue could apply."""
+        own, because a pixel's mean and variance are no per-channel scale and shift that the next conv's prologue could apply.  `src` is read
+        again by the reverse walk: no later op may overwrite it; other ops may read it.  A caller that puts a gradient of its own into src's
+        gradient buffer (a network output) needs a second reader on record, a `copy` for one: a sole reader's gradient is stored, not added."""
         if ln.normalized_shape != (src.c,) or any(p is not None and p.dtype != torch.float32 for p in (ln.weight, ln.bias)):
             raise ValueError("layer norm over %s in %s for %d channels" % (ln.normalized_shape, None if ln.weight is None else ln.weight.dtype, src.c))
         n, h, w, c = src.shape
