@@ -522,27 +522,32 @@ template <int DT, int GT, int T, int NV, int V> __global__ __launch_bounds__(T *
 
 // The workgroups' column sums: 32 columns a workgroup, 32 lanes down each, joined in LDS.  16 loads in flight a lane: 4 us for 512 workgroups'
 // sums, 6 with one.
+constexpr int JOINWG = 1 << 20;      // 2^30 lanes: a launch has fewer than 2^32.  Wider rows (above 2^24 values) take several turns
 __global__ __launch_bounds__(1024) void ln_bwd_join(LnJoinArgs a) {
   __shared__ float red[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;     // columns of {dw, db} side by side
-  float s = 0.f;
-  if (col < 2 * a.stride) {
+  const int part = threadIdx.x >> 5;
+  for (int c0 = blockIdx.x * 32; c0 < 2 * a.stride; c0 += JOINWG * 32) {
+    const int col = c0 + (threadIdx.x & 31);               // columns of {dw, db} side by side
+    float s = 0.f;
+    if (col < 2 * a.stride) {
 #pragma unroll 16
-    for (int b = part; b < a.blocks; b += 32) s += a.wpart[(long long)b * 2 * a.stride + col];
-  }
-  red[part][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (part == 0 && col < 2 * a.stride) {
-    s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) s += red[k][threadIdx.x];
-    const int i = col < a.stride ? col : col - a.stride;
-    void* out = col < a.stride ? a.dgamma : a.dbeta;
-    if (out && i < a.c) {
-      if (a.wdt == FD_F32) El<FD_F32>::store1(out, i, a.accumulate ? El<FD_F32>::load1(out, i) + s : s);
-      else if (a.wdt == FD_F16) El<FD_F16>::store1(out, i, a.accumulate ? El<FD_F16>::load1(out, i) + s : s);
-      else El<FD_BF16>::store1(out, i, a.accumulate ? El<FD_BF16>::load1(out, i) + s : s);
+      for (int b = part; b < a.blocks; b += 32) s += a.wpart[(long long)b * 2 * a.stride + col];
     }
+    red[part][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (part == 0 && col < 2 * a.stride) {
+      s = 0.f;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) s += red[k][threadIdx.x];
+      const int i = col < a.stride ? col : col - a.stride;
+      void* out = col < a.stride ? a.dgamma : a.dbeta;
+      if (out && i < a.c) {
+        if (a.wdt == FD_F32) El<FD_F32>::store1(out, i, a.accumulate ? El<FD_F32>::load1(out, i) + s : s);
+        else if (a.wdt == FD_F16) El<FD_F16>::store1(out, i, a.accumulate ? El<FD_F16>::load1(out, i) + s : s);
+        else El<FD_BF16>::store1(out, i, a.accumulate ? El<FD_BF16>::load1(out, i) + s : s);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -715,6 +720,10 @@ Shape shape_bwd(long long rows, long long c, int V) {
 }
 
 constexpr long long MAXC = 1ll << 29, MAXROWS = 1ll << 40;      // twice the columns is an int; row times pitch a long long
+constexpr long long MAXPIECES = 1ll << 24;                      // of all rows: a workgroup of 256 lanes each, and a launch has fewer than 2^32 lanes
+
+// split rows whose pieces are more than one launch takes
+bool too_many(const Shape& s, long long rows) { return s.T == 0 && rows >= (MAXPIECES + s.pieces - 1) / s.pieces; }
 
 bool known(int dt) { return dt == FD_F32 || dt == FD_F16 || dt == FD_BF16; }
 int esize(int dt) { return dt == FD_F32 ? 4 : 2; }
@@ -775,7 +784,6 @@ template <int DT> int launch_fwd(LnFwdArgs& a, hipStream_t st) {
     });
   a.piece = s.piece, a.pieces = s.pieces;
   const long long wgs = a.rows * s.pieces;
-  FD_REQUIRE(wgs < (1ll << 31), "layer_norm_fwd: %lld pieces", wgs);
   auto both = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
     const int rc = fd_launch(&ln_fwd_part<DT, NV>, "layer_norm_fwd_part", dim3((unsigned)wgs), dim3(256), 0, a, st);
@@ -797,7 +805,6 @@ template <int DT, int GT> int launch_bwd(LnBwdArgs& a, float* ws, const Shape& s
   a.part = ws;
   if (a.wpart) a.wpart = ws + ((2 * a.rows * s.pieces + 3) & ~3ll);
   const long long wgs = a.rows * s.pieces;
-  FD_REQUIRE(wgs < (1ll << 31), "layer_norm_bwd: %lld pieces", wgs);
   auto both = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
     if (a.dx) {
@@ -814,9 +821,10 @@ template <int DT, int GT> int launch_bwd(LnBwdArgs& a, float* ws, const Shape& s
 extern "C" int64_t fdgan_layer_norm_workspace(int64_t rows, int64_t c, int backward) {
   if (rows < 0 || rows > MAXROWS || c < 1 || c > MAXC) return -1;
   if (rows == 0) return 0;
-  long long most = 0;
+  long long most = -1;
   for (int V : {4, 8}) {
     const Shape s = backward ? shape_bwd(rows, c, V) : shape_fwd(rows, c, V);
+    if (too_many(s, rows)) continue;      // (the other types' vectors hold more)
     const long long f = s.floats > 0 ? s.floats + 4 : 0;
     most = f > most ? f : most;
   }
@@ -835,6 +843,7 @@ extern "C" int fdgan_layer_norm_fwd(const FdTensor* x, const void* gamma, const 
   if (rows == 0) return FD_OK;
   FD_REQUIRE(x->ptr != y->ptr, "layer_norm_fwd: y is x");
   const Shape s = shape_fwd(rows, x->c, x->dtype == FD_F32 ? 4 : 8);
+  FD_REQUIRE(!too_many(s, rows), "layer_norm_fwd: %lld rows of %lld values are too many for one call", rows, (long long)x->c);
   FD_REQUIRE(s.floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= s.floats), "layer_norm_fwd: a workspace of %lld floats at a multiple of 16 bytes", s.floats);
   LnFwdArgs a{x->ptr, y->ptr, gamma, beta, mean, rstd, ws, rows, px, py, (int)x->c, wdtype, 0, 0, eps, 1.f / (float)x->c};
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -863,6 +872,7 @@ extern "C" int fdgan_layer_norm_bwd(const FdTensor* x, const FdTensor* dy, const
   Shape s{};
   if (rows > 0) {
     s = shape_bwd(rows, x->c, x->dtype == FD_F32 ? 4 : 8);
+    FD_REQUIRE(!too_many(s, rows), "layer_norm_bwd: %lld rows of %lld values are too many for one call", rows, (long long)x->c);
     FD_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= s.floats + 4, "layer_norm_bwd: a workspace of %lld floats at a multiple of 16 bytes", s.floats + 4);
     LnBwdArgs a{x->ptr, dy->ptr, dx ? dx->ptr : nullptr, gamma, mean, rstd, nullptr, weights ? ws : nullptr, rows, px, pdy, pdx, (int)x->c, wdtype, 0, 0, 0, 0,
                 1.f / (float)x->c};
@@ -877,5 +887,6 @@ extern "C" int fdgan_layer_norm_bwd(const FdTensor* x, const FdTensor* dy, const
   }
   if (!weights) return FD_OK;
   LnJoinArgs j{ws, dgamma, dbeta, s.blocks, (int)x->c, s.stride, wdtype, accumulate ? 1 : 0};
-  return fd_launch(&ln_bwd_join, "layer_norm_bwd_join", dim3((unsigned)((2ll * s.stride + 31) / 32)), dim3(1024), 0, j, st);
+  const long long wgs = (2ll * s.stride + 31) / 32;
+  return fd_launch(&ln_bwd_join, "layer_norm_bwd_join", dim3((unsigned)(wgs < JOINWG ? wgs : JOINWG)), dim3(1024), 0, j, st);
 }

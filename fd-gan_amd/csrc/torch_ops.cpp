@@ -97,6 +97,7 @@ Result forward_rows(const Tensor& x, const Tensor& w, const Tensor& b, int64_t l
   r.x = in.t;
   const FdTensor out{r.y.data_ptr(), rows, 1, 1, c, {c, c, c, 1}, in.fd.dtype, 0};
   const int64_t floats = entries.workspace(rows, c, 0);
+  TORCH_CHECK_VALUE(floats >= 0, "layer_norm: ", rows, " rows of ", c, " values are too many for one call");
   const Tensor ws = floats > 0 ? at::empty({floats}, x.options().dtype(at::kFloat)) : Tensor();
   float* mean = keep ? r.stats.data_ptr<float>() : nullptr;
   const Tensor& wt = w.defined() ? w : b;
@@ -144,6 +145,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
         const Rows rx = rows_of(x, lead, c, rows), rdy = rows_of(dy, lead, c, rows);
         const Tensor w = weight.defined() ? weight.contiguous() : weight;
         const int64_t floats = entries.workspace(rows, c, 1);
+        TORCH_CHECK_VALUE(floats >= 0, "layer_norm: the gradients of ", rows, " rows of ", c, " values are too many for one call");
         const Tensor ws = at::empty({floats}, x.options().dtype(at::kFloat));
         const FdTensor dx{ptr(out[0]), rows, 1, 1, c, {c, c, c, 1}, rx.fd.dtype, 0};
         const float* mean = stats.data_ptr<float>();

@@ -525,7 +525,8 @@ int fdgan_adam_step_clipped(float* p, const float* g, float* m, float* v, int64_
  *   fdgan_layer_norm_fwd    mean / rstd: one fp32 per row for the backward pass (NULL: not kept)
  *   fdgan_layer_norm_bwd    dy and dx of x's dtype, or FD_BF16 gradients of FD_F16 activations; dx NULL: not wanted.  dgamma / dbeta: `c`
  *                           values of wdtype, NULL: not wanted; accumulate != 0 adds to what they hold (else it is overwritten).
- * Outputs do not overlap inputs.  ws: fdgan_layer_norm_workspace(rows, c, backward) floats (0: none needed). */
+ * Outputs do not overlap inputs.  ws: fdgan_layer_norm_workspace(rows, c, backward) floats (0: none needed;
+ * below 0: rows above 2^40, c above 2^29, or long rows -- c above 6144 -- of more than 2^24 pieces of 1024 to 8192 values in all). */
 int64_t fdgan_layer_norm_workspace(int64_t rows, int64_t c, int backward);
 int fdgan_layer_norm_fwd(const FdTensor* x, const void* gamma, const void* beta, int wdtype, float eps, const FdTensor* y, float* mean,
                          float* rstd, float* ws, int64_t ws_floats, FdStream stream);
