@@ -161,8 +161,8 @@ template <class Fn> __device__ __forceinline__ void each_stretch(const SpanTable
   }
 }
 
-// Bound by memory: 348 MB of bf16 in 81 us (4.3 TB/s), with half of it still behind the L2s from the pass before; 268 MB of fp32 in 82 us read
-// through the caches and in 45 us (6 TB/s) past them.  The start of a workgroup (finding its tensor) and its join cost 3 to 4 us, which is what
+// Bound by memory: 348 MB of bf16 in 87 us (4.0 TB/s), with half of it still behind the L2s from the pass before; 268 MB of fp32 in 82 us read
+// through the caches and in 44 us (6 TB/s) past them.  The start of a workgroup (finding its tensor) and its join cost 3 to 4 us, which is what
 // lists of a few MB take.
 constexpr int NT = 512;               // lanes of a workgroup of the norm pass
 
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256) void norm_finish_kernel(FinishArgs a) {
   }
 }
 
-// 348 MB of bf16 read and written in 120 us (5.8 TB/s).  The factor is formed by every workgroup for itself: 1000 partials are 8 KB from the L2,
+// 348 MB of bf16 read and written in 131 us (5.3 TB/s).  The factor is formed by every workgroup for itself: 1000 partials are 8 KB from the L2,
 // 1 to 2 us, where a launch between the passes would cost 3 to 4.
 template <int DT> __device__ __forceinline__ void scale_share(void* p, long long i, long long end, float f) {
   constexpr int V = El<DT>::V;
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(ScaleArgs a) {
   });
 }
 
-// 67 million parameters: 28 bytes each in 361 us (5.2 TB/s); 790416: 6 us, of which the factor is 2.
+// 67 million parameters: 28 bytes each in 368 us (5.1 TB/s); 790416: 6 us, of which the factor is 2.
 template <bool PAST> __device__ __forceinline__ f32x4 get4(const float* p) {
   return PAST ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)) : *reinterpret_cast<const f32x4*>(p);
 }

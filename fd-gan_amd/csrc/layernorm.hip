@@ -5,7 +5,8 @@
 //              dx = s (g - c1 - h c2),   dw = sum over rows of dy h,   db = sum over rows of dy
 //
 // A row is a pixel of an NHWC view (C channels, next to each other; the rows may lie at a pitch wider than C, a channel slice of a
-// concatenation) or a row of a matrix.  Sums are in fp32; the variance is formed around the mean, never as a difference of squares.
+// concatenation) or a row of a matrix.  Sums are in fp32; the variance is formed around the mean (or around a value some roundings beside it, and
+// what that adds is taken off: mend_mean), never as a difference of the squares of x.
 //
 // All of it is bound by memory: 2 C or 3 C values a row against some 10 to 20 operations a value.  So each value is read once:
 //  * held rows (ln_fwd_rows, ln_bwd_rows): a row stays in the registers of a group of T lanes, NV vectors of 16 bytes each.  T is a power of
@@ -209,8 +210,8 @@ __device__ __forceinline__ float around(float mean_square, float e) {
 }
 
 // ---- forward, held rows ---------------------------------------------------------------------------------------------------------
-// Bound by memory: 45.5 us for 128 MB in and out (65536 x 1024 bf16, 5.9 TB/s; a copy of 128 MB runs at 7.2, one of 2 GB at 4.9), 48 us for
-// 16384 x 4096 bf16, 17 us for 262144 x 72 fp16 (4.4 TB/s: rows of 144 bytes end inside lines).  Two or three vectors a lane because one
+// Bound by memory: 46 us for 128 MB in and out (65536 x 1024 bf16, 5.8 TB/s; a copy of 128 MB runs at 7.2, one of 2 GB at 4.9), 50 us for
+// 16384 x 4096 bf16, 17.6 us for 262144 x 72 fp16 (4.3 TB/s: rows of 144 bytes end inside lines).  Two or three vectors a lane because one
 // leaves lanes idle: 24 us instead of 17 at 72 channels, 16 lanes of which 9 work.
 template <int DT, int T, int NV> __global__ __launch_bounds__(block_of<T>()) void ln_fwd_rows(LnFwdArgs a) {
   constexpr int V = El<DT>::V, R = block_of<T>() / T;      // rows of a workgroup at a time
@@ -300,7 +301,7 @@ template <int DT, int T, int NV> __global__ __launch_bounds__(block_of<T>()) voi
 // ---- forward, split rows --------------------------------------------------------------------------------------------------------
 // A piece is 256 lanes x NV vectors.  The first pass leaves each piece's own mean and its sum of squares around that mean; the second
 // joins a row's pieces (mean of the means by their lengths; squares around the pieces' means plus the means' own around the row's) and
-// applies the norm.  x is read twice, the second time from a cache where it fits one.  8 rows of 196608 fp32: 3.2 + 4.7 us, against 946 us
+// applies the norm.  x is read twice, the second time from a cache where it fits one.  8 rows of 196608 fp32: 3.2 + 4.8 us, against 946 us
 // for one workgroup a row; both are a launch and one round of memory latency.
 template <int DT, int NV> __global__ __launch_bounds__(256) void ln_fwd_part(LnFwdArgs a) {
   constexpr int V = El<DT>::V;
@@ -386,7 +387,8 @@ template <int DT, int NV> __global__ __launch_bounds__(256) void ln_fwd_apply(Ln
 // ---- backward, held rows --------------------------------------------------------------------------------------------------------
 // An element that does not exist has dy = 0 and h = 0 and so adds nothing anywhere.  What waits for a row's two sums are the vectors as they were
 // loaded, converted a second time: half the registers of the converted ones, which is what decides how many waves a CU holds.
-// 82 us for 16384 x 4096 bf16 (402 MB, 4.9 TB/s: a large copy's rate), 52 us for 262144 x 144 fp16 (4.4 TB/s).
+// 84 us for 16384 x 4096 bf16 (402 MB, 4.8 TB/s: a large copy's rate), 52 us for 262144 x 144 fp16 (4.3 TB/s; the same with bf16 gradients), 33 for
+// 262144 x 72 (3.4).
 // Rows of T lanes: one vector a lane up to 512 of them (few registers, many waves), two or three only where a row takes all 512.
 template <int T> constexpr int bwd_rows_of() { return T > 256 ? 1 : T > 128 ? 2 : T == 128 ? 4 : 512 / T; }      // a power of two: the sets are joined in halves
 template <int DT, int GT, int T, int NV, int V> __global__ __launch_bounds__(T * bwd_rows_of<T>()) void ln_bwd_rows(LnBwdArgs a) {
@@ -521,7 +523,7 @@ template <int DT, int GT, int T, int NV, int V> __global__ __launch_bounds__(T *
 }
 
 // The workgroups' column sums: 32 columns a workgroup, 32 lanes down each, joined in LDS.  16 loads in flight a lane: 4 us for 512 workgroups'
-// sums, 6 with one.
+// sums, 6 with one.  Few sets of many columns leave most lanes idle: 51 us for one set of 196608, more than the passes that made it.
 constexpr int JOINWG = 1 << 20;      // 2^30 lanes: a launch has fewer than 2^32.  Wider rows (above 2^24 values) take several turns
 __global__ __launch_bounds__(1024) void ln_bwd_join(LnJoinArgs a) {
   __shared__ float red[32][33];
@@ -552,6 +554,8 @@ __global__ __launch_bounds__(1024) void ln_bwd_join(LnJoinArgs a) {
 }
 
 // ---- backward, split rows -------------------------------------------------------------------------------------------------------
+// x and dy are read in both passes: 72 + 74 us for 4096 x 16384 fp16 (the passes' own reads and writes at 3.7 and 5.5 TB/s), 30 + 37 us for
+// 1024 x 16384 fp32.
 template <int DT, int GT, int NV> __global__ __launch_bounds__(256) void ln_bwd_part(LnBwdArgs a) {
   constexpr int V = El<DT>::V;
   __shared__ float red[2][16][2];
@@ -711,7 +715,8 @@ Shape shape_bwd(long long rows, long long c, int V) {
   if (rows * ((n + 511) / 512) < 512) s.NV = 1;
   s.piece = 256 * s.NV * V;
   s.pieces = (int)((c + s.piece - 1) / s.piece);
-  // rows of a workgroup: at least 8 (each leaves 2 floats a column behind, against the 6 to 12 bytes a value of every row), as many as leave the chip full
+  // rows of a workgroup: at least 8 (each workgroup leaves 2 floats a column behind, against the 6 to 12 bytes a value of every row), more where 1024
+  // workgroups have them.  Few long rows are few workgroups: 8 x 196608 fp32 are 96 of them, 10 us for the 19 MB of that pass
   long long slab = rows * s.pieces / 1024;
   s.slab = (int)(slab < 8 ? 8 : slab > MAXSLAB ? MAXSLAB : slab);
   s.blocks = (int)((rows + s.slab - 1) / s.slab);
