@@ -98,6 +98,7 @@ class FlatAdam:
             with torch.cuda.device(self.flat.device):
                 L.check(L.load().fdgan_adam_step(self.flat.data_ptr(), self.grad.data_ptr(), self.m.data_ptr(), self.v.data_ptr(), self.flat.numel(),
                                                  lr, self.betas[0], self.betas[1], self.eps, self.t, E.stream_ptr()), "adam_step")
+            self.grad_norm = None
         else:
             self.grad_norm = adam_step_(self.flat, self.grad, self.m, self.v, self.t, lr, self.betas, self.eps, self.max_norm)
         # the kernel wrote the parameters behind autograd's back: bump their version counters, which is what the

@@ -96,3 +96,7 @@ def test_an_optimizer_without_a_bound_needs_the_library_alone(O, monkeypatch):
     a.step()
     assert a.grad_norm is None and ps[0]._version > version
     assert torch.equal(a.flat, b.flat) and torch.equal(a.m, b.m) and torch.equal(a.v, b.v)
+    assert b.grad_norm is not None
+    b.max_norm = None                                      # the bound is taken off: no norm of an earlier step stays behind
+    b.step()
+    assert b.grad_norm is None
