@@ -847,6 +847,8 @@ class D(_PlannedModule):
     norm (ours): "batch" is the reference's network; "layer" has a layer norm over each pixel's channels in the two BatchNorms' places
     (`ln` instead of `bn` in the state_dict keys), so that an image's map does not depend on the others in its batch."""
 
+    norm = "batch"      # of modules that were pickled whole before there was a choice
+
     def __init__(self, nc, nf, norm="batch"):
         super().__init__()
         if norm not in ("batch", "layer"):
