@@ -444,6 +444,7 @@ extern "C" int fdgan_adam_step(float* p, const float* g, float* m, float* v, int
                                float eps, int64_t step, FdStream stream) {
   FD_REQUIRE(p && g && m && v && n > 0 && step >= 1, "adam_step: bad arguments");
   FD_REQUIRE((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) == 0, "adam_step: 16-byte aligned flat tensors");
+  FD_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adam_step: betas %g, %g (0 <= beta < 1)", beta1, beta2);
   AdamArgs a{p, m, v, g, n, adam_constants(lr, beta1, beta2, eps, step)};
   return fd_launch(&adam_kernel, "adam_step", dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, a, static_cast<hipStream_t>(stream));
 }

@@ -453,6 +453,7 @@ extern "C" int fdgan_adam_step_clipped(float* p, const float* g, float* m, float
                                        int64_t step, float max_norm, double* partial, int64_t capacity, float* norm_out, FdStream stream) {
   FD_REQUIRE(p && g && m && v && n > 0 && step >= 1, "adam_step_clipped: bad arguments");
   FD_REQUIRE((((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v) & 15) == 0, "adam_step_clipped: 16-byte aligned flat tensors");
+  FD_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adam_step_clipped: betas %g, %g (0 <= beta < 1)", beta1, beta2);
   FD_REQUIRE(norm_out && partial && max_norm >= 0.f, "adam_step_clipped: NULL output or workspace, or max_norm %g", (double)max_norm);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const FdGradSpan s{const_cast<float*>(g), n, FD_F32};

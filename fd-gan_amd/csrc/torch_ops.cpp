@@ -295,6 +295,7 @@ std::optional<Tensor> adam_step(const Tensor& p, const Tensor& g, const Tensor& 
   const char* at[4] = {static_cast<char*>(p.data_ptr()), static_cast<char*>(g.data_ptr()), static_cast<char*>(m.data_ptr()), static_cast<char*>(v.data_ptr())};
   std::sort(at, at + 4);
   for (int k = 1; k < 4; ++k) TORCH_CHECK_VALUE(n == 0 || at[k] - at[k - 1] >= 4 * n, "adam_step_: two of the tensors share memory");
+  TORCH_CHECK_VALUE(b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1, "adam_step_: betas ", b1, ", ", b2, " (0 <= beta < 1)");
   TORCH_CHECK_VALUE(step >= 1, "adam_step_: step ", step, " (counts from 1)");
   TORCH_CHECK_VALUE(!max_norm || *max_norm >= 0, "adam_step_: max_norm ", max_norm.value_or(0));
   at::NoGradGuard off;

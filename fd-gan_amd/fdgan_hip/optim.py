@@ -57,6 +57,8 @@ class FlatAdam:
         every rank) and leaves that norm, from before clipping, in `grad_norm` -- a 0-dim device tensor, not read back here."""
         if max_norm is not None and not max_norm >= 0.0:
             raise ValueError("FlatAdam: max_norm %r" % (max_norm,))
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("FlatAdam: betas %r (0 <= beta < 1)" % (tuple(betas),))
         self.max_norm, self.grad_norm = max_norm, None
         self.params = [p for p in params if p.requires_grad]
         if not self.params:

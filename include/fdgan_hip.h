@@ -491,7 +491,7 @@ int fdgan_grad_ew(int mode, const FdTensor* src, const FdTensor* ref, const FdTe
 
 /* torch.optim.Adam's update (no weight decay, no amsgrad -- what the reference's lrG / lrD / beta1 flags configure,
  * demo.py:43-46) on one flat fp32 tensor: exp_avg m, exp_avg_sq v, 1-based `step` for the bias corrections.  The betas are
- * doubles (ABI v18): 1 - beta and 1 - beta^step are formed from them in 64 bits and rounded once. */
+ * doubles (ABI v18), 0 <= beta < 1: 1 - beta and the bias corrections are formed from them in 64 bits and rounded once. */
 int fdgan_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float lr, double beta1, double beta2, float eps,
                     int64_t step, FdStream stream);
 
